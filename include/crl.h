@@ -119,8 +119,8 @@ int crl_attn_decode(const void* q, int64_t q_bs, const void* k, int64_t k_bs, in
  * the rows of a head (row_s = 64, head_s = page_size * 64: the faster one).  page_size: a power of two up to 4096.  A sequence covers
  * max_pages * page_size positions.  lengths, starts, counts (int32) and the page table live on the device: a captured graph serves every step.
  * A page id outside [0, n_pages) or a length outside [0, max_pages * page_size] is never followed: attention writes NaN to that sequence's
- * rows of o (and, for a page, adds NaN to its weights), append drops the row, evict leaves the sequence as it is.  Pages that a call writes (the page of an appended token, the pages of
- * an evicted sequence) must belong to one sequence; pages that are only read may be shared.
+ * rows of o (and, for a page, adds NaN to its weights), append drops the row, evict leaves the whole sequence as it is.  Pages that a call writes
+ * (the page of an appended token, the pages of an evicted sequence) must belong to one sequence; pages that are only read may be shared.
  *
  * crl_paged_attn_decode: o[b, h] = softmax(scale q[b, h] . K[b, h / (H / Hkv)]) V over the lengths[b] positions of sequence b; a length of 0
  * gives zeros.  k_new / v_new (optional, [B, Hkv * 64]): the row of position lengths[b] - 1 comes from here and is written to its page by
@@ -147,7 +147,8 @@ int crl_paged_append(const void* k, int64_t k_bs, int64_t k_rs, const void* v, i
 /* Cuts every sequence longer than `budget` down to it, per key-value head: the last `recent` positions stay, and of the others those with the
  * largest weights (equal weights: the lower position; NaN above all numbers), in their order, moved down to positions 0 .. budget - 1 in
  * place together with their weights.  Positions from `budget` on keep what they held.  new_lengths[b] = min(lengths[b], budget) (may be
- * lengths itself); kept (optional, [B, Hkv, budget] int32): the positions that stayed, in order, -1 behind the last.
+ * lengths itself); kept (optional, [B, Hkv, budget] int32): the positions that stayed, in order, -1 behind the last.  A sequence whose length lies
+ * outside its table, or that would be cut and has a page outside the pool under one of its positions, keeps rows, weights and length; its kept is -1.
  * ws >= crl_cache_evict_ws_bytes(B, Hkv, budget), with kept given crl_cache_evict_ws_bytes(B, Hkv, 0). */
 size_t crl_cache_evict_ws_bytes(int B, int Hkv, int budget);
 int crl_cache_evict(void* k_pages, void* v_pages, int64_t page_s, int64_t row_s, int64_t head_s, int n_pages, int page_size,

@@ -407,7 +407,7 @@ struct EvictArgs {
   int* new_lengths;
   float* weights; int64_t w_bs, w_hs;
   int* kept;                            // [B * Hkv][budget]
-  int* moved;                           // [B * Hkv] rows that the second launch moves
+  int* moved;                           // [B * Hkv] rows that the second launch moves: budget, or 0 for a sequence that stays as it is
   int B, Hkv, budget, recent;
 };
 
@@ -516,11 +516,10 @@ __device__ __forceinline__ void move_tile(const Pages& pg, const int* table, u16
   }
 }
 
-__device__ __forceinline__ int cut_length(const EvictArgs& a, int n) { return n < 0 || n > a.pg.cap ? n : min(n, a.budget); }
-
 // One workgroup per (sequence, key-value head).  The `need`-th largest weight among the old positions by a radix selection (digits of 11, 11
 // and 10 bits, histogram in LDS), then one ordered pass that writes the kept positions and moves their weights down.  A thread holds up to 8
 // neighbouring positions in registers; a sequence of up to 8192 is read once.  Integer atomics only: the result does not depend on their order.
+// The page ids are looked over while the weights are on their way, in the barrier that the empty histogram needs anyway: no time of its own.
 // MOVE: the same workgroup then moves the rows of K and V.  Bound by the rounds of the selection (read, three histograms, the ordered pass; each waits
 // for the one before): 11.5 us for 128 heads of 6189 positions, whose 3.2 MB take under 1; with MOVE, 96 heads of 1023 that keep 512, 13.4 us.
 template <bool MOVE>
@@ -532,14 +531,13 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const EvictArgs a) {
   const int bh = blockIdx.x, b = bh / a.Hkv, h = bh % a.Hkv;
   const int n = a.lengths[b];
   int* kept = a.kept + (int64_t)bh * a.budget;
-  const bool bad = n < 0 || n > a.pg.cap;
-  if (MOVE && h == 0 && tid == 0) a.new_lengths[b] = cut_length(a, n);
-  if (bad || n <= a.budget) {
+  const int* table = a.pg.table + b * a.pg.table_ld;
+  const auto leave = [&](int stay) {    // the sequence as it is; of the list, its first `stay` positions
+    if (MOVE && h == 0 && tid == 0) a.new_lengths[b] = n;
     if (!MOVE && tid == 0) a.moved[bh] = 0;
-    for (int i = tid; i < a.budget; i += SEL) kept[i] = (!bad && i < n) ? i : -1;
-    return;
-  }
-  if (!MOVE && tid == 0) a.moved[bh] = a.budget;
+    for (int i = tid; i < a.budget; i += SEL) kept[i] = i < stay ? i : -1;
+  };
+  if (n < 0 || n > a.pg.cap || n <= a.budget) { leave(n > a.pg.cap ? 0 : n); return; }
   float* w = a.weights + b * a.w_bs + h * a.w_hs;
   const int old = n - a.recent;         // recent <= budget < n
   uint32_t need = a.budget - a.recent;  // how many of the old ones stay
@@ -554,9 +552,20 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const EvictArgs a) {
   };
   const bool once = n <= tile;
   if (once) load(0);
+  // one page outside the pool leaves the whole sequence as it is: every head of it looks at the same entries and finds the same
+  bool off = false;
+  for (int i = tid; i <= (n - 1) >> a.pg.shift; i += SEL) off |= (unsigned)table[i] >= (unsigned)a.pg.n_pages;
+  const bool off_wave = __any(off);
+  if ((tid & 63) == 0) sh[1][tid >> 6] = off_wave;
+  for (int i = tid; i < RN; i += SEL) hist[i] = 0;
+  __syncthreads();
+  uint32_t off_any = 0;
+#pragma unroll
+  for (int i = 0; i < SEL / 64; ++i) off_any |= sh[1][i];
+  if (off_any) { leave(0); return; }
+  if (MOVE && h == 0 && tid == 0) a.new_lengths[b] = a.budget;
+  if (!MOVE && tid == 0) a.moved[bh] = a.budget;
   if (some) {
-    for (int i = tid; i < RN; i += SEL) hist[i] = 0;
-    __syncthreads();
     for (int pass = 0; pass < 3; ++pass) {
       const int sft = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t bins = pass == 2 ? 1 << 10 : RN;
@@ -617,7 +626,6 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const EvictArgs a) {
   }
   if (MOVE) {
     __syncthreads();                    // the list is complete
-    const int* table = a.pg.table + b * a.pg.table_ld;
     u16 *k = a.k + h * a.pg.head_s, *v = a.v + h * a.pg.head_s;
     if (a.budget <= MTILE) {
       move_tile(a.pg, table, k, v, hist, a.budget);
@@ -632,8 +640,8 @@ __global__ __launch_bounds__(SEL) void evict_select_kernel(const EvictArgs a) {
 template <int LPR>
 __global__ __launch_bounds__(SEL) void evict_move_kernel(const EvictArgs a) {
   const int bh = blockIdx.x, b = bh / a.Hkv, h = bh % a.Hkv;
-  if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lengths[b] = cut_length(a, a.lengths[b]);
   const int count = a.moved[bh];
+  if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lengths[b] = count ? count : a.lengths[b];
   if (count == 0) return;
   move_rows<LPR>(a.pg, a.pg.table + b * a.pg.table_ld, (blockIdx.y & 1 ? a.v : a.k) + h * a.pg.head_s + 8 * LPR * (blockIdx.y >> 1),
                  a.kept + (int64_t)bh * a.budget, count);

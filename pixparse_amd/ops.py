@@ -451,7 +451,7 @@ def cache_evict(k_pages, v_pages, page_table, lengths, weights, budget: int, rec
     others, those with the largest weights (weights [B, kv_heads, positions] fp32, as paged_attn_decode gathers them; equal ones: the lower
     position) move to positions 0 .. budget - 1, in order, in place, with their weights.  new_lengths [B] int32 (may be lengths itself)
     receives min(lengths, budget); kept [B, kv_heads, budget] int32 (optional) the positions that stayed, -1 behind the last.  The pages of
-    a sequence must be its own."""
+    a sequence must be its own.  A sequence with a length outside the table, or one to be cut with a page outside the pool, stays whole (kept: -1)."""
     tn, ts, sh, ks = page_table.shape, page_table.stride(), k_pages.shape, k_pages.stride()
     B, index = tn[0], k_pages.get_device()
     ws = weights.stride() if weights is not None else None
