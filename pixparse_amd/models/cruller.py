@@ -418,10 +418,11 @@ class Cruller(nn.Module):
         self-attention cache in pages (layers/paged_cache.py).  encoder_outputs [B, S, D]; prompts: B lists of token ids (any lengths, B not
         limited by the 16 rows of the contiguous cache).  Every sequence ends at its own eos_id (kept) or after max_steps tokens.
 
-        self_budget: the self-attention cache holds at most self_budget + evict_every positions a head; every evict_every steps it is cut to
-        self_budget -- the last self_recent (default: a quarter) and those that gathered the most attention.  cross_budget: after
-        cross_after steps the encoder tokens of every layer and head are cut to the cross_budget that were attended to most.  Both trade
-        exactness for memory and time; without them the tokens are those of the uncut cache.
+        self_budget: every evict_every steps the self-attention cache is cut to self_budget positions a head -- the last self_recent (default: a
+        quarter) and those to which the tokens generated so far gave the most attention.  It holds at most self_budget + evict_every positions a
+        head, and a longer prompt whole, with evict_every more, until its first cut.  cross_budget: after cross_after steps the encoder tokens of every
+        layer and head are cut to the cross_budget that were attended to most.  Both trade exactness for memory and time;
+        without them the tokens are those of the uncut cache.
 
         Returns a list of B dicts: 'ids' (the generated tokens), 'logprob' and 'entropy' (fp32, one per token: its log probability, and the
         entropy of the distribution it was taken from), 'top_ids' / 'top_logprob' [n, top]."""
@@ -445,7 +446,7 @@ class Cruller(nn.Module):
         cut_self = self_budget is not None and max(lens) + max_steps > self_budget
         cut_cross = cross_budget is not None and cross_budget < S
         positions = [n - 1 + max_steps for n in lens]
-        if cut_self:       # a prompt longer than the budget is held whole until the first cut, which follows the prefill
+        if cut_self:       # a prompt longer than the budget is held whole until the first cut: before the first steps there are no weights to cut it by
             positions = [min(p, max(n - 1, self_budget) + evict_every) for p, n in zip(positions, lens)]
         enc16 = encoder_outputs.reshape(B * S, D).to(torch.bfloat16).contiguous()
         dec.paged_begin(enc16, B, S, positions, page_size, weights=cut_self, cross_weights=cut_cross)
@@ -481,8 +482,6 @@ class Cruller(nn.Module):
             return min(evict_every - done % evict_every if cut_self else max_steps, cross_after - done if cross is not None and done < cross_after else max_steps)
 
         done, graph = 0, None
-        if cut_self:
-            cache.evict(self_budget, recent)
         while done < max_steps and not (done and bool(finished.all())):
             n = min(check_every, max_steps - done, due(done))
             for _ in range(n):

@@ -1,0 +1,56 @@
+"""Scores of given tokens and their backward pass, and the cuts of a bounded cache, through the model on a real MI355X."""
+import pytest
+import torch
+
+from tests.test_model_paged_gpu import PROMPTS, build
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device('cuda:0')
+
+
+def test_a_prompt_is_cut_by_the_attention_it_got(dev, monkeypatch):
+    """A prompt longer than the budget is held whole until attention weights exist: up to the first regular cut the tokens are those of the uncut run,
+    their scores up to the bf16 policy's tolerance.  At that cut every one of the 8 steps has given every head weights of sum 1: base-2 scores under 64
+    less their maximum round by 2^-18 at most, once for the sum and once for the weight, v_exp by 2^-22, 43 additions by 2^-18 in all: within 2^-16
+    of 1.  It keeps the positions that the definition keeps, which are not the lowest everywhere."""
+    from pixparse_amd.layers import paged_cache
+    model, _, _, image, _, _ = build(dev)
+    enc = model.image_encoder(image.to(dev)).clone()
+    long = [p * 3 for p in PROMPTS]                        # 36, 3 and 15 tokens
+    budget, recent, every, steps = 16, 6, 8, 20
+    plain = model.generate_paged(enc, long, -1, steps)
+    cuts = []
+    evict = paged_cache.PagedCache.evict
+
+    def spy(self, b, r):
+        before = [w.clone() for w in self.weights], self.lengths.clone()
+        k = [t.clone() for t in self.k]
+        evict(self, b, r)
+        cuts.append((before, [t.clone() for t in self.k], k, self.table.clone()))
+    monkeypatch.setattr(paged_cache.PagedCache, 'evict', spy)
+    got = model.generate_paged(enc, long, -1, steps, self_budget=budget, self_recent=recent, evict_every=every)
+    for a, b in zip(got, plain):
+        assert a['ids'][:every] == b['ids'][:every]
+        assert float((a['logprob'][:every] - b['logprob'][:every]).abs().max()) <= 2 * 3e-2 * max(1.0, float(b['top_logprob'].abs().max()))
+        assert len(a['ids']) == steps and bool(torch.isfinite(a['logprob']).all())
+    (weights, lengths), after, k, table = next(c for c in cuts if int(c[0][1].max()) > budget)
+    assert lengths.tolist() == [len(p) - 1 + every for p in long]
+    n = int(lengths[0])
+    lowest = list(range(budget - recent)) + list(range(n - recent, n))
+    others = 0
+    for layer, w in enumerate(weights):
+        for h in range(w.shape[1]):
+            x = w[0, h, :n].double().cpu()
+            assert abs(float(x.sum()) - every) <= every * 2 ** -16
+            at = sorted(sorted(range(n - recent), key=lambda p: (-float(x[p]), p))[:budget - recent]) + list(range(n - recent, n))
+            others += at != lowest
+            size = k[layer].shape[1]
+            row = lambda pool, p: pool[layer][int(table[0, p // size]), p % size, h]
+            for i, p in enumerate(at):
+                assert torch.equal(row(after, i), row(k, p))
+    assert others > 0
