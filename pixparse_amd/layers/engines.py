@@ -472,7 +472,9 @@ class BartEngine(_Base):
         # is switched on.  Sites: 0 = embedding LayerNorm output, 1 + 3 i + {0, 1, 2} = self-attention /
         # cross-attention / fc2 branch of layer i before its residual join (modeling_bart.py:362,377,384-386,654).
         self.drop: Optional[ops.DropSpec] = None
-        self.scored = None                # (B, T) between Cruller.forward_logprobs and backward_logprobs: the logits buffer still holds the logits
+        # (B, T) from Cruller.forward_logprobs on: the logits buffer holds logits; () once another encoder pass has replaced the activations behind
+        # them; None after backward_logprobs or another forward
+        self.scored = None
 
     def _hidden_drop(self):
         return self.drop is not None and self.drop.p > 0

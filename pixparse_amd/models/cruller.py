@@ -278,9 +278,11 @@ class Cruller(nn.Module):
 
     # ------------------------------------------------------------------ compute
     def encode(self, image_input: torch.Tensor):
-        enc, _, _ = self._ensure_engines()
+        enc, dec, _ = self._ensure_engines()
         assert image_input.shape[1:] == (self.in_chans, *self.img_size), \
             f'image {tuple(image_input.shape)} does not match the configured {self.in_chans}x{self.img_size}'  # timm strict img size
+        if dec.scored:                # the encoder's activations become this pass's: no backward_logprobs() of an earlier one
+            dec.scored = ()
         enc32, enc16 = enc.forward(image_input.contiguous().float())
         return enc32, enc16
 
@@ -529,10 +531,11 @@ class Cruller(nn.Module):
     def backward_logprobs(self, d_logprob: Optional[torch.Tensor], d_entropy: Optional[torch.Tensor] = None,
                           on_ready: Optional[Callable[[str], None]] = None, first_micro: bool = False):
         """backward() of the last forward_logprobs() for the gradients of an objective with respect to its two results (fp32 [B, T], either may be
-        None): weight gradients accumulate into arena.g as in backward().  Once: the gradient takes the place of the logits."""
+        None): weight gradients accumulate into arena.g as in backward().  Once, and with no other pass of the encoder or decoder in between (generation
+        from encoder outputs at hand is none): the gradient takes the place of the logits."""
         _, dec, bufs = self._ensure_engines()
-        if dec.scored is None:
-            raise RuntimeError('backward_logprobs() continues from the forward_logprobs() right before it, once')
+        if not dec.scored:
+            raise RuntimeError('backward_logprobs() continues from the forward_logprobs() right before it, once, with no other pass of the model in between')
         for name, t in (('d_logprob', d_logprob), ('d_entropy', d_entropy)):
             if t is not None and t.shape != dec.scored:
                 raise ValueError(f'{name}: expected shape {dec.scored}, got {tuple(t.shape)}')
@@ -570,6 +573,8 @@ class Cruller(nn.Module):
         enc, dec, bufs = self._ensure_engines()
         enc.first_micro = dec.first_micro = bool(first_micro) and _WGRAD_OVERWRITE
         assert self.arena.g is not None, 'call alloc_training_state() (train_setup) before backward'
+        if dec.scored is not None:    # the logits buffer holds logits, not their gradient
+            raise RuntimeError('backward() continues from forward_loss(); after forward_logprobs() it is backward_logprobs()')
         S = enc.out_tokens()
         denc = bufs.get('denc', (dec.B * S, dec.D), torch.float32)     # written (not accumulated) by the decoder's last layer first
         dec.backward(bufs.t['dec.logits'], bufs.t[enc.tag + '.norm.y16'], denc, on_ready)

@@ -13,6 +13,15 @@ def dev():
     return torch.device('cuda:0')
 
 
+def training(dev, seed=12):
+    from oracle import ref_cpu as R
+    model, _, _, image, tokens, target = build(dev, L=32, B=2, seed=seed)
+    ti, tt = R.shift_tokens(tokens, target)
+    model.arena.alloc_training_state()
+    model.arena.g.zero_()
+    return model, image.to(dev), ti.to(dev).clone(), tt.to(dev).clone()
+
+
 def test_a_prompt_is_cut_by_the_attention_it_got(dev, monkeypatch):
     """A prompt longer than the budget is held whole until attention weights exist: up to the first regular cut the tokens are those of the uncut run,
     their scores up to the bf16 policy's tolerance.  At that cut every one of the 8 steps has given every head weights of sum 1: base-2 scores under 64
@@ -54,3 +63,28 @@ def test_a_prompt_is_cut_by_the_attention_it_got(dev, monkeypatch):
             for i, p in enumerate(at):
                 assert torch.equal(row(after, i), row(k, p))
     assert others > 0
+
+
+def test_no_gradient_through_another_forward(dev):
+    """an encoder pass in between leaves its own activations behind, and a plain backward() has no logit gradients to start from: both are refused
+    before a gradient is touched, and what is still sound goes on"""
+    model, image, ti, tt = training(dev)
+    d = torch.full(tt.shape, -0.1, device=dev)
+    model.forward_logprobs(image, ti, tt)
+    model.backward_logprobs(d)
+    want = model.arena.g.clone()
+    model.arena.g.zero_()
+    for between in (lambda: model.image_encoder(image.flip(0)), lambda: model.encode_image(image[:1]), lambda: model.encode(image)):
+        model.forward_logprobs(image, ti, tt)
+        between()
+        for backward in (lambda: model.backward_logprobs(d), model.backward):
+            with pytest.raises(RuntimeError, match='forward_logprobs'):
+                backward()
+    model.forward_logprobs(image, ti, tt)
+    with pytest.raises(RuntimeError, match='backward_logprobs'):
+        model.backward()
+    assert not bool(model.arena.g.any())
+    model.backward_logprobs(d)
+    assert torch.equal(model.arena.g, want)
+    model.forward_loss(image, ti, tt)
+    model.backward()
