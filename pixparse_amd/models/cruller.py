@@ -517,16 +517,18 @@ class Cruller(nn.Module):
     # ------------------------------------------------------------------ scores of given tokens, and training on them
     def forward_logprobs(self, image_input, text_input, text_target):
         """forward() and, for every target token, its log probability (-100: 0), and the entropy of every row's distribution, those with target -100
-        too: (logprob [B, T], entropy [B, T]) fp32.  backward_logprobs() continues from here; a caller that only scores need not call it."""
+        too: (logprob [B, T], entropy [B, T]) fp32, the caller's own.  backward_logprobs() continues from here; a caller that only scores need not
+        call it."""
         _, dec, bufs = self._ensure_engines()
         self.forward(image_input, text_input)
         B, T = text_input.shape
         logits = bufs.t['dec.logits']
-        self._target = text_target.contiguous().view(-1)
-        logprob, entropy, lse = (bufs.get('score.' + n, (B * T,), torch.float32) for n in ('logprob', 'entropy', 'lse'))
+        self._target = text_target.reshape(-1).clone()               # (targets and entropy as they are now: backward_logprobs reads both)
+        logprob = torch.empty(B * T, dtype=torch.float32, device=logits.device)
+        entropy, lse = (bufs.get('score.' + n, (B * T,), torch.float32) for n in ('entropy', 'lse'))
         ops.token_logprobs(logits, self._target, self.vocab_size, logprob, entropy=entropy, lse=lse)
         dec.scored = (B, T)
-        return logprob.view(B, T), entropy.view(B, T)
+        return logprob.view(B, T), entropy.clone().view(B, T)
 
     def backward_logprobs(self, d_logprob: Optional[torch.Tensor], d_entropy: Optional[torch.Tensor] = None,
                           on_ready: Optional[Callable[[str], None]] = None, first_micro: bool = False):

@@ -88,3 +88,23 @@ def test_no_gradient_through_another_forward(dev):
     assert torch.equal(model.arena.g, want)
     model.forward_loss(image, ti, tt)
     model.backward()
+
+
+def test_scores_belong_to_the_caller(dev):
+    """the next call leaves them alone; changing them, or the targets, in place changes no gradient"""
+    model, image, ti, tt = training(dev)
+    logprob, entropy = model.forward_logprobs(image, ti, tt)
+    kept = logprob.clone(), entropy.clone()
+    d = torch.linspace(-1, 1, tt.numel(), device=dev).view(tt.shape)
+    model.backward_logprobs(d, 0.1 * d)
+    want = model.arena.g.clone()
+    other = model.forward_logprobs(image.flip(0), ti, tt)
+    assert torch.equal(logprob, kept[0]) and torch.equal(entropy, kept[1])
+    assert not torch.equal(other[0], logprob) and not torch.equal(other[1], entropy)
+    model.arena.g.zero_()
+    logprob, entropy = model.forward_logprobs(image, ti, tt)
+    logprob.zero_()
+    entropy.fill_(7.0)
+    tt.fill_(3)
+    model.backward_logprobs(d, 0.1 * d)
+    assert torch.equal(model.arena.g, want) and bool(want.any())
