@@ -520,6 +520,8 @@ class Cruller(nn.Module):
         too: (logprob [B, T], entropy [B, T]) fp32, the caller's own.  backward_logprobs() continues from here; a caller that only scores need not
         call it."""
         _, dec, bufs = self._ensure_engines()
+        if text_target.shape != text_input.shape:
+            raise ValueError(f'text_target: expected shape {tuple(text_input.shape)}, that of text_input, got {tuple(text_target.shape)}')
         self.forward(image_input, text_input)
         B, T = text_input.shape
         logits = bufs.t['dec.logits']

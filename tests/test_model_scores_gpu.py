@@ -108,3 +108,10 @@ def test_scores_belong_to_the_caller(dev):
     tt.fill_(3)
     model.backward_logprobs(d, 0.1 * d)
     assert torch.equal(model.arena.g, want) and bool(want.any())
+
+
+def test_targets_of_another_shape_are_refused(dev):
+    model, image, ti, tt = training(dev)
+    for bad in (tt.t(), tt.reshape(-1), tt[:, :-1]):
+        with pytest.raises(ValueError, match='text_target'):
+            model.forward_logprobs(image, ti, bad)
