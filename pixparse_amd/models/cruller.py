@@ -287,7 +287,7 @@ class Cruller(nn.Module):
         return enc32, enc16
 
     def set_train_dropout(self, enabled: bool, seed: int = 0):
-        """Opt-in hidden-state dropout of the text decoder inside forward_loss() / backward(): the reference's
+        """Opt-in hidden-state dropout of the text decoder inside forward_loss() / backward() and forward_logprobs() / backward_logprobs(): the reference's
         decoder runs it only when built with pretrained=False (BartForCausalLM from_config stays in train mode, p = config.dropout;
         text_decoder_hf.py:25-33); parity runs, bench.py and every eval / generation path keep it off.  The mask of micro-step s is
         a pure function of (seed, s, site, element) -- crl_dropout in include/crl.h.  Covers all four train-mode regularisers of the
@@ -299,6 +299,13 @@ class Cruller(nn.Module):
         p_path = float(self.enc_arch.get('drop_path', 0.0)) if self.enc_kind == 'swin' else 0.0   # timm Swin drop-path (train-mode encoder)
         self._drop = (p, int(seed), p_attn, p_act, p_path) if enabled and max(p, p_attn, p_act, p_path) > 0 else None
         self._drop_step = 0
+
+    def _next_drop(self) -> Optional[ops.DropSpec]:
+        """the masks of the next training micro-step, None where dropout is off"""
+        if getattr(self, '_drop', None) is None:
+            return None
+        self._drop_step += 1
+        return ops.DropSpec(self._drop[0], self._drop[1], self._drop_step - 1, *self._drop[2:])
 
     def forward(self, image_input: torch.Tensor, text_input: torch.Tensor, _drop=None):
         """ref models/cruller.py:14-21 -> output['logits'] bf16 [B, T, V] (a view of the padded logits buffer)."""
@@ -515,14 +522,16 @@ class Cruller(nn.Module):
         return result
 
     # ------------------------------------------------------------------ scores of given tokens, and training on them
-    def forward_logprobs(self, image_input, text_input, text_target):
+    def forward_logprobs(self, image_input, text_input, text_target, dropout: bool = True):
         """forward() and, for every target token, its log probability (-100: 0), and the entropy of every row's distribution, those with target -100
         too: (logprob [B, T], entropy [B, T]) fp32, the caller's own.  backward_logprobs() continues from here; a caller that only scores need not
-        call it."""
+        call it.  Like forward_loss() it runs as one training micro-step under the dropout that set_train_dropout() has switched on, if any;
+        dropout=False: without, for scores of the model as it generates."""
         _, dec, bufs = self._ensure_engines()
         if text_target.shape != text_input.shape:
             raise ValueError(f'text_target: expected shape {tuple(text_input.shape)}, that of text_input, got {tuple(text_target.shape)}')
-        self.forward(image_input, text_input)
+        self._scored_drop = self._next_drop() if dropout else None
+        self.forward(image_input, text_input, _drop=self._scored_drop)
         B, T = text_input.shape
         logits = bufs.t['dec.logits']
         self._target = text_target.reshape(-1).clone()               # (targets and entropy as they are now: backward_logprobs reads both)
@@ -547,6 +556,7 @@ class Cruller(nn.Module):
         flat = lambda t: None if t is None else t.contiguous().view(-1)
         ops.token_logprobs_bwd(logits, self._target, self.vocab_size, bufs.t['score.lse'], bufs.t['score.entropy'], flat(d_logprob), flat(d_entropy), logits)
         dec.scored = None
+        dec.drop = self._scored_drop          # (generation in between has switched it off)
         self.backward(on_ready, first_micro)
 
     def forward_loss(self, image_input, text_input, text_target, loss_mul: float = 1.0, grad_mul: float = 1.0,
@@ -554,11 +564,7 @@ class Cruller(nn.Module):
         """forward + shifted-token cross-entropy; leaves d(loss*grad_mul)/dlogits in the logits buffer.
         returns the device scalar loss (fp32, = mean NLL * loss_mul)."""
         enc, dec, bufs = self._ensure_engines()
-        drop = None
-        if getattr(self, '_drop', None) is not None:
-            drop = ops.DropSpec(self._drop[0], self._drop[1], self._drop_step, *self._drop[2:])
-            self._drop_step += 1
-        self.forward(image_input, text_input, _drop=drop)   # dec.drop stays set for the matching backward()
+        self.forward(image_input, text_input, _drop=self._next_drop())   # dec.drop stays set for the matching backward()
         B, T = text_input.shape
         M = B * T
         logits = bufs.t['dec.logits']

@@ -115,3 +115,36 @@ def test_targets_of_another_shape_are_refused(dev):
     for bad in (tt.t(), tt.reshape(-1), tt[:, :-1]):
         with pytest.raises(ValueError, match='text_target'):
             model.forward_logprobs(image, ti, bad)
+
+
+def test_training_on_scores_uses_the_configured_dropout(dev):
+    """the masks of forward_loss() at the same micro-step, in both directions, also where tokens are generated in between; none with dropout=False.
+    (The bounds are those of the comparison without dropout: one bf16 rounding of either logit gradient, 2^-8 of a gradient, and half as much
+    again for the roundings of the backward pass.)"""
+    model, image, ti, tt = training(dev)
+    n = int((tt != -100).sum())
+    clean = model.forward_logprobs(image, ti, tt)
+    enc = model.image_encoder(image).clone()
+    model.dec_arch = dict(model.dec_arch, dropout=0.25)
+    model.set_train_dropout(True, seed=5)
+    loss = float(model.forward_loss(image, ti, tt))
+    model.backward()
+    want = model.arena.g.clone()
+    for generate in (False, True):
+        model.set_train_dropout(True, seed=5)
+        model.arena.g.zero_()
+        logprob, entropy = model.forward_logprobs(image, ti, tt)
+        assert abs(float(-logprob.sum() / n) - loss) <= 1e-5 * max(1.0, loss)
+        if generate:
+            model.generate_paged(enc, [[3, 4], [5]], -1, 3)
+        model.backward_logprobs(torch.full_like(logprob, -1.0 / n))
+        for name, e in model.arena.entries.items():
+            a, b = model.arena.grad(name).float(), want[e.offset:e.offset + e.numel].view_as(model.arena.grad(name))
+            assert float((a - b).norm()) <= 3 * 2 ** -8 * float(b.norm()), name
+    # micro-steps count on as forward_loss() does: the next masks are others
+    assert not torch.equal(model.forward_logprobs(image, ti, tt)[0], logprob)
+    same = model.forward_logprobs(image, ti, tt, dropout=False)
+    assert torch.equal(same[0], clean[0]) and torch.equal(same[1], clean[1])
+    model.set_train_dropout(False)
+    same = model.forward_logprobs(image, ti, tt)
+    assert torch.equal(same[0], clean[0]) and torch.equal(same[1], clean[1])
