@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const u16* k, const u
   const int count = min(counts[b], T), start = starts[b];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int t = (int)(i / (Hkv * 8)), r = (int)(i % (Hkv * 8)), h = r >> 3, part = r & 7;
-  if (t >= count || start < 0 || start > pg.cap - 1 - t) return;
+  if (t >= count || start > pg.cap - 1 - t || start < -t) return;        // (no sum that could pass 32 bits)
   const int p = start + t;
   int64_t to;
   if (!row_of(pg, pg.table + b * pg.table_ld, p, to)) return;
