@@ -719,6 +719,9 @@ extern "C" int crl_paged_attn_decode(const void* q, int64_t q_s, void* k_pages, 
   a.B = B; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.nsub = (a.group + HEADS - 1) / HEADS; a.scale = scale;
   CRL_CHECK((int64_t)B * Hkv * a.nsub < (1ll << 31) && (int64_t)B * H < (1ll << 31), "%s: too many sequences", who);
   a.nsplit = paged_plan(B * Hkv * a.nsub, a.nsub, a.group, a.pg.cap, weights != nullptr);
+  const bool join_weights = weights && (a.nsplit > 1 || a.nsub > 1);
+  const int wblocks = (a.pg.cap + 1023) / 1024;              // 1024 positions each of the joining launch
+  CRL_CHECK(!join_weights || wblocks + a.group < 65536, "%s: weights of %d positions and %d query heads a key-value head are too many", who, a.pg.cap, a.group);
   const size_t want = crl_paged_attn_decode_ws_bytes(B, H, Hkv, page_size, max_pages, weights != nullptr);
   CRL_CHECK(want == 0 || (ws && ws_bytes >= want), "%s: workspace too small (%zu bytes, %zu needed)", who, ws_bytes, want);
   a.ws = (float*)ws;
@@ -738,9 +741,7 @@ extern "C" int crl_paged_attn_decode(const void* q, int64_t q_s, void* k_pages, 
   if (wide) { if (weights) paged_attn_kernel<8, true><<<grid, 512, 0, s>>>(a); else paged_attn_kernel<8, false><<<grid, 512, 0, s>>>(a); }
   else { if (weights) paged_attn_kernel<4, true><<<grid, 256, 0, s>>>(a); else paged_attn_kernel<4, false><<<grid, 256, 0, s>>>(a); }
   CRL_LAUNCH_CHECK(who);
-  if (weights && (a.nsplit > 1 || a.nsub > 1)) {
-    const int wblocks = (a.pg.cap + 1023) / 1024;
-    CRL_CHECK(wblocks + a.group < 65536, "%s: a sequence's table covers too many positions", who);
+  if (join_weights) {
     paged_join_weights_kernel<<<dim3((unsigned)(B * Hkv), (unsigned)(wblocks + a.group)), 256, 0, s>>>(a, wblocks);
     CRL_LAUNCH_CHECK("crl_paged_attn_decode(join, weights)");
   } else if (a.nsplit > 1) {
