@@ -435,13 +435,13 @@ class Cruller(nn.Module):
 
         Returns a list of B dicts: 'ids' (the generated tokens), 'logprob' and 'entropy' (fp32, one per token: its log probability, and the
         entropy of the distribution it was taken from), 'top_ids' / 'top_logprob' [n, top]."""
-        _, dec, bufs = self._ensure_engines()
-        dec.drop = None
         dev, B, V = self.device, encoder_outputs.shape[0], self.vocab_size
         if len(prompts) != B or any(len(p) < 1 for p in prompts):
             raise ValueError(f'{B} images need {B} prompts of one token or more')
         if max_steps < 1 or not 1 <= top <= min(32, V):
             raise ValueError(f'max_steps {max_steps}: 1 or more; top {top}: 1 to 32')
+        if check_every < 1:
+            raise ValueError(f'check_every {check_every}: 1 or more')
         lens = [len(p) for p in prompts]
         if max(lens) + max_steps > self.max_length:
             raise ValueError(f'{max(lens)} prompt tokens and {max_steps} steps exceed the {self.max_length} learned positions')
@@ -452,6 +452,8 @@ class Cruller(nn.Module):
         S, D = encoder_outputs.shape[1:]
         if cross_budget is not None and (cross_budget < 1 or cross_after < 1):
             raise ValueError(f'cross_budget {cross_budget}, cross_after {cross_after}')
+        _, dec, bufs = self._ensure_engines()
+        dec.drop = None
         cut_self = self_budget is not None and max(lens) + max_steps > self_budget
         cut_cross = cross_budget is not None and cross_budget < S
         positions = [n - 1 + max_steps for n in lens]
