@@ -60,8 +60,9 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __
 // (g = lane >> 4) and its output channels 16 c + 4 g + r, so maximum, sum and rescaling never leave it but for the maximum over the four g.
 // K rows, then V rows go through the wave's own 8 KiB of LDS (16-byte chunks at chunk ^ (row & 7)), whole rows of memory an instruction, and come
 // back as operands: K by rows, V transposed (ds_read_b64_tr_b16).  The key order of P V is that of the scores' registers: P needs no exchange.
-// The probabilities enter P V as the sum of two bf16 numbers, the second under 2^-7 of the whole: off by 2^-15 of themselves, an error that the
-// bf16 rounding of the output (2^-8) hides.  All else is fp32.
+// The probabilities enter P V as the sum of two bf16 numbers of their sign.  The first is 0.9961 p rounded, by half a step (2^-8) at most: under p.  The
+// second is the rest, over 0 and up to 2^-7 of p, rounded by 2^-8 of itself: p is off by 2^-15 of itself at most, which the bf16 rounding of the
+// output (2^-8) hides.  Neither is 0 or negative where p is not (down to 2^-109, where the rest is a normal number still), so an infinite value gives infinity.  All else is fp32.
 // Bound by the key and value rows, read once from HBM and by nobody again: 8 sequences of 24935 keys, 16 heads: 818 MB in 143 us, 5.7 TB/s
 // (random 8 KiB reads alone reach 5.85, a copy of 1 GB 5.05); 32 sequences of up to 6189 keys, 16 query heads on 4: 102 MB in 22 us.  The latter's
 // vector units have 16 scores per key to exponentiate; where heads share keys, the matrix cores take the products from them (with dot products on the
@@ -192,8 +193,8 @@ __global__ __launch_bounds__(64 * NW, W ? 3 : 4) void paged_attn_kernel(const Pa
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float p = s[2 * u + (j >> 2)][j & 3];
-        hi[j] = (__bf16)(p * 0.998f);
-        lo[j] = (__bf16)(p - (float)hi[j]);                  // > 0 wherever p is: an infinite value row must meet no 0
+        hi[j] = (__bf16)(p * 0.9961f);                       // 0.9961 (1 + 2^-8) < 1: never rounded up to p, so the rest is over 0
+        lo[j] = (__bf16)(p - (float)hi[j]);
       }
 #pragma unroll
       for (int cg = 0; cg < 4; ++cg) {
