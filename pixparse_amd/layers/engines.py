@@ -719,7 +719,7 @@ class BartEngine(_Base):
     def paged_begin(self, enc16: torch.Tensor, B: int, S: int, positions, page_size: int = 64, weights: bool = False, cross_weights: bool = False):
         """decode_begin with the self-attention cache in pages (PagedCache): sequences at lengths of their own, any number of them; positions[b] =
         the most positions sequence b will hold; weights: gather attention weights for its eviction.  cross_weights: the cross-attention cache in
-        pages as well, gathering weights."""
+        pages as well, gathering weights, beside the contiguous one that decode_prefill reads."""
         dp, D = self.DP, self.D
         pos = self.buf('gen.positions', (B,), torch.int32)
         pos.zero_()

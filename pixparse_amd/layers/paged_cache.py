@@ -53,6 +53,6 @@ class PagedCache:
         self.lengths.copy_(self._cut)
 
     def freeze(self, positions: int) -> None:
-        """from now on no sequence holds more than `positions`: the table ends there, and no more weights are gathered"""
+        """from now on no sequence holds more than `positions`: the table ends there, and no more weights are gathered (the pools keep their size)"""
         self.table = self.table[:, :-(-positions // self.page_size)].contiguous()
         self.weights = [None] * len(self.weights)

@@ -430,8 +430,10 @@ class Cruller(nn.Module):
         self_budget: every evict_every steps the self-attention cache is cut to self_budget positions a head -- the last self_recent (default: a
         quarter) and those to which the tokens generated so far gave the most attention.  It holds at most self_budget + evict_every positions a
         head, and a longer prompt whole, with evict_every more, until its first cut.  cross_budget: after cross_after steps the encoder tokens of every
-        layer and head are cut to the cross_budget that were attended to most.  Both trade exactness for memory and time;
-        without them the tokens are those of the uncut cache.
+        layer and head are cut to the cross_budget that were attended to most.  Both trade exactness for time; without them the tokens are those of
+        the uncut cache.  self_budget also bounds the pages of the self-attention cache, which are laid out once, for the most a sequence may reach (one
+        that has ended keeps its pages, and computes on, until all have).  cross_budget takes memory instead: the encoder's keys and values of every
+        layer stand in pages beside the contiguous ones that the prompt reads, and the cut gives none back.
 
         Returns a list of B dicts: 'ids' (the generated tokens), 'logprob' and 'entropy' (fp32, one per token: its log probability, and the
         entropy of the distribution it was taken from), 'top_ids' / 'top_logprob' [n, top]."""
