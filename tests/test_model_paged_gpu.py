@@ -111,7 +111,7 @@ def test_budgets(dev):
         assert len(x['ids']) == 30 and bool(torch.isfinite(x['logprob']).all()) and x['ids'][:5] == y['ids'][:5]
     cache, cross = model._engines[1].gen['cache'], model._engines[1].gen['cross']
     assert all(16 <= n <= 24 for n in cache.lengths.tolist()) and cross.lengths.tolist() == [S // 2] * 3
-    long = [p * 3 for p in PROMPTS]                     # a prompt of 36 tokens is cut to the budget before the first step
+    long = [p * 3 for p in PROMPTS]                     # a prompt of 36 tokens is cut to the budget after eight steps
     c = model.generate_paged(enc, long, -1, 12, **cut)
     assert all(len(x['ids']) == 12 and bool(torch.isfinite(x['logprob']).all()) for x in c)
 

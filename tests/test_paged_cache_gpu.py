@@ -108,8 +108,8 @@ SHAPES = [
     (2, 12, 12, 8, [63, 64], 'qkv'),
     (4, 4, 4, 64, [65, 0, 128, 200], 'head'),
     (2, 16, 4, 32, [300, 257], 'row'),
-    (2, 6, 2, 16, [511, 30], 'head'),           # three query heads a key-value head: the fourth slot of its workgroup is empty
-    (1, 20, 2, 16, [77], 'qkv'),                # ten: two workgroups, the second of two heads
+    (2, 6, 2, 16, [511, 30], 'head'),           # three query heads a key-value head, of the 16 that a workgroup takes
+    (1, 20, 2, 16, [77], 'qkv'),                # ten
     (2, 8, 1, 128, [1025, 1024], 'head'),       # eight, split over the length
     (3, 2, 1, 64, [2049, 0, 1], 'row'),         # two, split, one sequence with fewer keys than splits
     (1, 1, 1, 256, [6189], 'head'),
