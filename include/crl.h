@@ -126,8 +126,9 @@ int crl_attn_decode(const void* q, int64_t q_bs, const void* k, int64_t k_bs, in
  * gives zeros.  k_new / v_new (optional, [B, Hkv * 64]): the row of position lengths[b] - 1 comes from here and is written to its page by
  * the same launch.  weights (optional, fp32, element (b, h, p) at b * w_bs + h * w_hs + p): the attention weights of the call are added at
  * every position, summed over the query heads that share the key-value head; the position of an appended token starts from 0.  Positions
- * at or behind the length keep their values.  Scores, sums, and the probabilities in P.V are fp32.  ws: >= crl_paged_attn_decode_ws_bytes
- * (which may be 0); calls that may run at the same time need workspaces of their own. */
+ * at or behind the length keep their values.  Scores, sums and accumulators are fp32; a probability enters P.V as the sum of two bf16 numbers, off by
+ * 2^-15 of itself at most (the output is rounded to bf16 by 2^-8).  ws: >= crl_paged_attn_decode_ws_bytes (which may be 0); calls that may run at
+ * the same time need workspaces of their own. */
 /* where the kernels look for a position: *offset = elements from the base to its row (head 0), for one row of a page table in HOST memory; 1 where
  * the table leads outside the pool or the position outside the table.  Host arithmetic only. */
 int crl_paged_row(const int* host_table_row, int position, int64_t page_s, int64_t row_s, int n_pages, int page_size, int max_pages,
@@ -377,7 +378,8 @@ int crl_cross_entropy(const void* logits, int64_t ldl, const int64_t* target, in
  * entropy; a row of nothing but -inf has no distribution: logprob, entropy and top_logprob NaN, lse -inf.  Rows with NaN or +inf: NaN.
  * crl_token_logprobs_bwd: dlogits (type of logits, row stride ldd, may be logits itself) =
  *   d_logprob[r] (1[j = target] - p_j) - d_entropy[r] p_j (log p_j + entropy[r]),  columns V..cols-1 zeroed;
- * lse and entropy as the forward call gave them; d_logprob / d_entropy optional, not both NULL.  A target of -100 takes no d_logprob; a row that
+ * lse and entropy as the forward call gave them: p_j = e^(x_j - lse) carries the rounding of lse, 2^-24 |lse| of itself, beside the bounds of the scores (which
+ * take deviations from the maximum and do not depend on a common offset of the logits); d_logprob / d_entropy optional, not both NULL.  A target of -100 takes no d_logprob; a row that
  * takes neither gradient (or zeros) becomes zeros, whatever its logits are. */
 int crl_token_logprobs(const void* logits, int is_f32, int64_t ldl, const int64_t* target, int64_t M, int V, float* logprob,
                        float* entropy, float* lse, int k, float* top_logprob, int64_t top_ld, int64_t* top_ids, int64_t ids_ld, void* stream);

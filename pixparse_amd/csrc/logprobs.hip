@@ -1,7 +1,8 @@
 // Log probabilities of given tokens, entropy, log-sum-exp and the k most probable tokens of rows of logits, and the gradient of the first
 // two (include/crl.h: crl_token_logprobs, crl_token_logprobs_bwd).
 //   m = max x, S = sum 2^t, T = sum t 2^t with t = (x - m) log2(e):  lse = m + ln S,  H = ln 2 (log2 S - T / S),  log p_j = (x_j - m) - ln S
-// all in fp32; the deviations t are taken before anything is summed, so neither H nor log p is a difference of large numbers.
+// all in fp32; the deviations t are taken before anything is summed, so neither H nor log p is a difference of large numbers.  The gradient takes log p_j
+// as x_j - lse: exact but for the rounding of lse to fp32, so log p, and relatively p, are off by 2^-24 |lse| there.
 #include "common.h"
 
 namespace {
