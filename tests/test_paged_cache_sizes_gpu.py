@@ -43,3 +43,18 @@ def test_more_query_heads_than_a_workgroup_takes(dev, B, H, kv, page, lengths, l
 ])
 def test_evict_long_sequences(dev, B, kv, page, lengths, layout, budget, recent, kind, in_place):
     paged.test_evict(dev, B, kv, page, lengths, layout, budget, recent, kind, in_place)
+
+
+@pytest.mark.parametrize('append', [False, True])
+@pytest.mark.parametrize('weights', [False, True])
+@pytest.mark.parametrize('H,kv,pages', [(4, 4, 20), (12, 2, 70), (2, 1, 2000)])
+def test_lengths_far_below_the_capacity(dev, H, kv, pages, append, weights, monkeypatch):
+    """a table that covers what sequences may still reach (320 to 32000 positions), most splits without a key; entries behind the length hold no page"""
+    made = paged.Case.__init__
+
+    def init(self, dev, B, H, kv, page, lengths, layout, seed=0):
+        made(self, dev, B, H, kv, page, lengths, layout, seed, pages=pages)
+        for b, n in enumerate(lengths):
+            self.table[b, -(-n // page):] = -1
+    monkeypatch.setattr(paged.Case, '__init__', init)
+    paged.test_paged_attention(dev, 5, H, kv, 16, [0, 1, 64, 130, 310], 'head', append, weights)
