@@ -129,8 +129,9 @@ __device__ __forceinline__ void shift(float& S, float& T, float from, float to) 
 }
 
 // One workgroup of NT threads per row.  A thread walks its 16-byte pieces U at a time, the next U on their way, with a maximum and sums of its
-// own: no barrier until the row has been read.  The logits are read once, and bound it: 8184 x 50304 bf16, 823 MB in 150 to 166 us, 5.0 to 5.5 TB/s
-// (a copy of that size reaches 5.05); 8 rows of 50267, 9.7 us, are latency: launch, 6 pieces a thread, three exchanges, the candidates' second look.
+// own: no barrier until the row has been read.  The logits are read once, and bound it: 8184 x 50304 bf16, 823 MB in 151 us, 5.45 TB/s
+// (a copy of that size reaches 5.05; the first hundred calls up to 190), without top tokens 147, with masked columns 178 to 195 (the exponentials of a
+// batch that holds a mask are computed twice); 8 rows of 50267, 9.9 us, are latency: launch, 6 pieces a thread, three exchanges, the candidates' second look.
 // The k best: the k-th largest of the maxima of 64 groups of lanes is a bound that the k-th best cannot be under.  The lanes whose maximum
 // reaches it (about k of them) read the pieces around it once more (all of theirs where the second largest reaches it too) and put what reaches it
 // into a list in LDS that the first wave picks from.  Rows of many equal values overflow the list and take k rounds over the row instead.
@@ -343,7 +344,8 @@ __device__ __forceinline__ u32x4 pack16(const float (&o)[8]) { return u32x4{pack
 __device__ __forceinline__ u32x4 pack16(const float (&o)[4]) { return u32x4{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])}; }
 
 // d x_j = g (1[j = t] - p_j) - gH p_j (log p_j + H); p_j = 0 takes its limit 0. one workgroup per row and 256 * BWD_U pieces; columns from V on zeroed.
-// lse and H are the forward's, so a logit needs no other: read once, written once.  8184 x 50304 bf16: 1.65 GB in 313 us, 5.26 TB/s
+// lse and H are the forward's, so a logit needs no other: read once, written once.  8184 x 50304 bf16: 1.65 GB in 315 us, 5.24 TB/s;
+// right behind the forward call, which leaves a part of the logits in the last cache, 280
 constexpr int BWD_U = 4;                // 16-byte loads in flight per thread
 template <typename T, bool FAR>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const LpBwdArgs a) {
@@ -424,8 +426,10 @@ extern "C" int crl_token_logprobs(const void* logits, int is_f32, int64_t ldl, c
   CRL_CHECK(k == 0 || (top_logprob && top_ids && top_ld >= k && ids_ld >= k), "%s: top_logprob and top_ids need %d columns", who, k);
   LpArgs a{logits, ldl, target, logprob, entropy, lse, top_logprob, top_ids, top_ld, ids_ld, M, V, k};
   hipStream_t s = as_stream(stream);
-  // Threads a row: a wave for short rows; 1024 where there are fewer rows than places for workgroups and only latency counts (8 rows of 50267:
-  // 9.7 us, with 256 threads 18); 256 elsewhere, eight rows a CU in different phases (8184 rows: 166 us, with 1024 threads 229)
+  // Threads a row: a wave for short rows; 1024 where there are fewer rows than places for workgroups and only latency counts; 256 elsewhere, eight rows
+  // a CU in different phases.  256 against 1024 threads, rows of 50267 bf16, the best token, in us: 8 rows 10.5 / 8.2, 128 11.3 / 9.0, 256 13.3 / 10.1,
+  // 384 15.1 / 14.7, 512 18.0 / 15.3, 768 21.5 / 22.8, 1024 25.2 / 28.2, 2048 45.3 / 50.7, 8184 151 / 175; 8 rows of 4096 4.8 / 4.7, 8192 5.2 / 5.2,
+  // 16384 6.1 / 5.7.
   const int pieces = (V + vec - 1) / vec;
   if (pieces <= 128) { if (is_f32) launch_lp<float, 64, 2>(a, s); else launch_lp<u16, 64, 2>(a, s); }
   else if (M >= 512 || pieces <= 1024) { if (is_f32) launch_lp<float, 256, 2>(a, s); else launch_lp<u16, 256, 2>(a, s); }
@@ -453,7 +457,8 @@ extern "C" int crl_token_logprobs_bwd(const void* logits, int is_f32, int64_t ld
   const dim3 grid((unsigned)M, (unsigned)(((cols + vec - 1) / vec + 256 * BWD_U - 1) / (256 * BWD_U)));
   CRL_CHECK(grid.y < 65536, "%s: too many columns (%d)", who, cols);
   // Past the caches where the logits are larger than the last of them (256 MiB): nobody finds a line again, and keeping them costs evictions
-  // (8184 x 50304 bf16: 313 us against 330; 127 x 50304 fp32, which the forward call has just brought in: both calls 19.8 against 18.8, so not there).
+  // (8184 x 50304 bf16: 315 us against 329, behind the forward call both together 425 against 488; 127 x 50304 fp32, both calls: 19.8 against 18.8 with
+  // three sets of logits in turn, 21.0 against 22.4 with twelve, so no rule there).
   const bool far = (size_t)M * ldl * (is_f32 ? 4 : 2) > (256u << 20);
   hipStream_t s = as_stream(stream);
   if (is_f32) { if (far) logprobs_bwd_kernel<float, true><<<grid, 256, 0, s>>>(a); else logprobs_bwd_kernel<float, false><<<grid, 256, 0, s>>>(a); }

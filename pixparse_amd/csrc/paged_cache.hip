@@ -63,11 +63,11 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __
 // The probabilities enter P V as the sum of two bf16 numbers of their sign.  The first is 0.9961 p rounded, by half a step (2^-8) at most: under p.  The
 // second is the rest, over 0 and up to 2^-7 of p, rounded by 2^-8 of itself: p is off by 2^-15 of itself at most, which the bf16 rounding of the
 // output (2^-8) hides.  Neither is 0 or negative where p is not (down to 2^-109, where the rest is a normal number still), so an infinite value gives infinity.  All else is fp32.
-// Bound by the key and value rows, read once from HBM and by nobody again: 8 sequences of 24935 keys, 16 heads: 818 MB in 143 us, 5.7 TB/s
+// Bound by the key and value rows, read once from HBM and by nobody again: 8 sequences of 24935 keys, 16 heads: 818 MB in 144 us, 5.7 TB/s
 // (random 8 KiB reads alone reach 5.85, a copy of 1 GB 5.05); 32 sequences of up to 6189 keys, 16 query heads on 4: 102 MB in 22 us.  The latter's
 // vector units have 16 scores per key to exponentiate; where heads share keys, the matrix cores take the products from them (with dot products on the
 // vector units that call took 46 us against 29).  Batches of 64 keys: the next batch's rows fly while this one is computed, 4 waves a SIMD.
-// With weights the scores go to memory as well (and the registers' limit is 3 waves a SIMD): 6189 keys, 8 x 16 heads, 42 us of the call's 48.
+// With weights the scores go to memory as well (and the registers' limit is 3 waves a SIMD): 6189 keys, 8 x 16 heads, 43 us of the call's 48.
 template <int NW, bool W>
 __global__ __launch_bounds__(64 * NW, W ? 3 : 4) void paged_attn_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[NW][8192];
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256) void paged_join_weights_kernel(const PagedArgs
 }
 
 // rows [b, t] -> position starts[b] + t, t < counts[b]; 16 bytes a thread, all loads independent.  64 rows of 16 sequences, 16 heads, 8.4 MB read
-// and written: 4.9 us, little over an empty launch
+// and written: 4 to 5 us, little over an empty launch
 __global__ __launch_bounds__(256) void paged_append_kernel(const u16* k, const u16* v, int64_t k_bs, int64_t k_rs, int64_t v_bs, int64_t v_rs,
                                                            u16* kp, u16* vp, const Pages pg, const int* starts, const int* counts,
                                                            float* weights, int64_t w_bs, int64_t w_hs, int T, int Hkv) {
@@ -520,7 +520,7 @@ __device__ __forceinline__ void move_tile(const Pages& pg, const int* table, u16
 // One workgroup per (sequence, key-value head).  The `need`-th largest weight among the old positions by a radix selection (digits of 11, 11
 // and 10 bits, histogram in LDS), then one ordered pass that writes the kept positions and moves their weights down.  A thread holds up to 8
 // neighbouring positions in registers; a sequence of up to 8192 is read once.  Integer atomics only: the result does not depend on their order.
-// The page ids are looked over while the weights are on their way, in the barrier that the empty histogram needs anyway: no time of its own.
+// The page ids are looked over while the weights are on their way, in the barrier that the empty histogram needs anyway: 0.2 us of 17 for 256 heads.
 // MOVE: the same workgroup then moves the rows of K and V.  Bound by the rounds of the selection (read, three histograms, the ordered pass; each waits
 // for the one before): 11.5 us for 128 heads of 6189 positions, whose 3.2 MB take under 1; with MOVE, 96 heads of 1023 that keep 512, 13.4 us.
 template <bool MOVE>
@@ -669,6 +669,15 @@ Pages pages_of(const int* table, int64_t table_ld, int64_t page_s, int64_t row_s
 
 // Splits of a sequence's capacity.  One (no joining launch, 3 to 4 us) where eight waves get through it in two or four batches each; with weights
 // only if the workgroup has all query heads and few scores to go over again.  Else 2048 workgroups, twice what is resident, of 256 keys or more.
+// One split against several, full sequences, in us:
+//   capacity                                512          1024          2048          4096
+//   12 workgroups                        5.3 / 7.6     7.6 / 7.7    12.2 / 8.3    20.9 / 9.7
+//   64 workgroups                        5.6 / 8.1     7.8 / 9.4    14.6 / 13.1   25.0 / 19.2
+//   256 workgroups                       9.3 / 12.7   14.7 / 18.4   26.6 / 30.6   49.1 / 53.4
+//   12 heads, weights                    6.6 / 8.6     9.7 / 9.0    15.8 / 9.2    27.0 / 9.9
+//   16 heads on 4 (32 wg), weights       7.3 / 9.0    10.2 / 9.5    16.4 / 10.6   34.4 / 14.6
+//   256 heads, weights                  11.1 / 13.9   18.4 / 21.3   33.3 / 34.1   61.6 / 62.8
+// The rule is on the right side but for 12 to 64 workgroups at its border (up to 1.5 us).
 int paged_plan(int blocks, int nsub, int group, int cap, bool weights) {
   if (cap <= (blocks >= 64 ? 2048 : 1024) && !(weights && (nsub > 1 || (int64_t)cap * group > W_DIRECT))) return 1;
   const int max_split = (cap + 255) / 256;
@@ -794,8 +803,12 @@ extern "C" int crl_cache_evict(void* k_pages, void* v_pages, int64_t page_s, int
   a.B = B; a.Hkv = Hkv; a.budget = budget; a.recent = recent;
   hipStream_t s = as_stream(stream);
   // One launch where a workgroup a head is enough for the rows too: few of them, or heads for every CU.  The lengths must not change under the
-  // other heads of a sequence, so not in place.  (16 heads that move 1024 rows: as fast as two launches on the GPU, 4 us less on the host; 128 heads
-  // of 2048 rows: 44 us against 35, so not there.)
+  // other heads of a sequence, so not in place.  One launch against two on the GPU (the second costs the host 4 us), half of the positions kept, in us:
+  //   rows kept          512          1024          2048
+  //   16 heads       11.1 / 11.2   14.0 / 13.0   26.7 / 17.5
+  //   128 heads      14.2 / 15.2   21.0 / 20.7   45.0 / 43.1
+  //   256 heads      18.6 / 23.7   39.0 / 42.4   76.1 / 77.8
+  //   512 heads      44.9 / 47.2   74.9 / 77.8   135.7 / 140.6
   const bool apart = (const char*)new_lengths + 4ll * B <= (const char*)lengths || (const char*)lengths + 4ll * B <= (const char*)new_lengths;
   if (apart && (budget <= MTILE || B * Hkv >= 256)) {
     evict_select_kernel<true><<<(unsigned)(B * Hkv), SEL, 0, s>>>(a);
